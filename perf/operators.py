@@ -16,7 +16,6 @@ program serves one model); activations, caches, histories and masks come from th
 from __future__ import annotations
 
 import collections
-import ctypes as C
 import math
 import sys
 from pathlib import Path
@@ -224,25 +223,8 @@ def prepare(case, seed):
     return state
 
 
-class _Hbm:
-    """An array of a cache in HBM, for torch.as_tensor."""
-
-    def __init__(self, address, shape, typestr):
-        self.__cuda_array_interface__ = {"data": (address, False), "shape": shape, "typestr": typestr,
-                                         "version": 2, "strides": None}
-
-
-def _views(cache):
-    """A cache's K and V codes [heads][positions][HD] and K and V scales, in its own memory."""
-    alloc, at = C.c_uint32(), [C.c_void_p() for _ in range(4)]
-    cache.lib.nd_kv_info(cache.handle, C.byref(alloc), *[C.byref(a) for a in at])
-    rows = (cache.kv_heads, alloc.value)
-    shapes = [(rows + (HD,), "|i1")] * 2 + [(rows, "<f4")] * 2
-    return [torch.as_tensor(_Hbm(a.value, *s), device=DEVICE) for a, s in zip(at, shapes)]
-
-
 def _adopt(case, data):
-    """The program's handles: caches with the codes of both sides, workspaces, output buffers."""
+    """The program's handles: caches filled position by position, workspaces, output buffers."""
     hip, kind = _backend(), case["kind"]
     nh = _program["lib"]
     if kind == "product":
@@ -254,11 +236,11 @@ def _adopt(case, data):
         b, h, hq = case["batch"], case["kv_heads"], case["kv_heads"] * case["rep"]
         prefix = nh.HipKvCache(hip, 1, h, max(1, case["prefix"]))
         mine = nh.HipKvCache(hip, 1, b * h, case["own"])
-        for cache, name in ((prefix, "prefix"), (mine, "own")):
-            if case[name]:
-                for view, part in zip(_views(cache), ("kc", "vc", "ks", "vs")):
-                    view.copy_(data[f"{name}_{part}"].view(view.shape))
         torch.cuda.synchronize()
+        for cache, name, count in ((prefix, "prefix", case["prefix"]), (mine, "own", case["own"])):
+            hip._check(hip.lib.nd_kv_store_d(hip.ctx, cache.handle, 0, 0, count,
+                                             data[name + "_k"].data_ptr(), data[name + "_v"].data_ptr(), None))
+        hip._check(hip.lib.nd_sync(hip.ctx))
         data["lengths32"] = data["lengths"].int()
         data["out"] = torch.empty((b, hq, HD), device=DEVICE)
         data["shared"] = nh.HipSharedAttention(hip, b, h, hq)
