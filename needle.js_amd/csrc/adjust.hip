@@ -45,6 +45,16 @@ struct Record {
 };
 static_assert(sizeof(Record) == 32, "record layout");
 
+// The workspace: a counter of the rows that have advanced (nd_advance_row) in a line of
+// its own, then every row's place, the same whatever the batch of a call, so that calls
+// of any size up to the workspace's may follow one another.  Counters are zero between
+// launches, records hold what the last launch left.
+struct RowSpace {
+  uint32_t arrived;  // workgroups of the row
+  uint32_t pad[kCounterStride - 1];
+  Record records[kMaxRecords];
+};
+
 template <int SCOPE>
 __device__ __forceinline__ void put(uint32_t* p, uint32_t v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, SCOPE);
@@ -135,7 +145,7 @@ template <bool SELECT, bool STORE, bool XL>
 __global__ __launch_bounds__(kThreads, 6) void adjust_kernel(
     const float* logits, uint32_t vocab, nd_logit_adjust p,
     const uint32_t* __restrict__ mask_all, float* out, uint32_t* __restrict__ ids,
-    double* __restrict__ logprobs, Record* __restrict__ records, uint32_t* __restrict__ counters,
+    double* __restrict__ logprobs, uint32_t* __restrict__ rows_done, RowSpace* __restrict__ space,
     nd_select_advance adv, uint32_t rows, uint32_t S) {
   constexpr int kScope = XL ? __HIP_MEMORY_SCOPE_WORKGROUP : __HIP_MEMORY_SCOPE_AGENT;
   // Of the segment's ids: how often the history names them (then the adjusted
@@ -395,14 +405,15 @@ __global__ __launch_bounds__(kThreads, 6) void adjust_kernel(
     }
     ids[r] = id;
     logprobs[r] = lp;
-    if (adv.tokens) nd_advance_row(adv, r, rows, id, lp, counters + (size_t)rows * kCounterStride);
+    if (adv.tokens) nd_advance_row(adv, r, rows, id, lp, rows_done);
   };
   if (S == 1) {
     if (t == 0) finish();
     return;
   }
+  RowSpace* const own = space + r;
   if (t == 0) {
-    uint32_t* rec = reinterpret_cast<uint32_t*>(records + (size_t)r * kMaxRecords + part);
+    uint32_t* rec = reinterpret_cast<uint32_t*>(own->records + part);
     put<kScope>(rec, __float_as_uint(best.v));
     put<kScope>(rec + 1, best.order);
     put<kScope>(rec + 2, __float_as_uint(mx));
@@ -411,16 +422,14 @@ __global__ __launch_bounds__(kThreads, 6) void adjust_kernel(
     put<kScope>(rec + 4, (uint32_t)bits);
     put<kScope>(rec + 5, (uint32_t)(bits >> 32));
     __builtin_amdgcn_s_waitcnt(0);  // the record has completed
-    uint32_t* counter = counters + (size_t)r * kCounterStride;
-    const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, kScope) == S - 1;
-    if (last) put<kScope>(counter, 0u);
+    const bool last = __hip_atomic_fetch_add(&own->arrived, 1u, __ATOMIC_RELAXED, kScope) == S - 1;
+    if (last) put<kScope>(&own->arrived, 0u);
     s_last = last;
   }
   __syncthreads();
   if (!s_last || w != 0) return;
 
-  const uint32_t* rec =
-      reinterpret_cast<const uint32_t*>(records + (size_t)r * kMaxRecords + (lane < S ? lane : 0));
+  const uint32_t* rec = reinterpret_cast<const uint32_t*>(own->records + (lane < S ? lane : 0));
   best = Best{__uint_as_float(get(rec)), get(rec + 1)};
   mx = __uint_as_float(get(rec + 2));
   key = get(rec + 3);
@@ -440,11 +449,11 @@ __global__ __launch_bounds__(kThreads, 6) void adjust_kernel(
 
 struct nd_selector {
   uint32_t batch = 0;
-  void* work = nullptr;  // records, then counters (zero between calls)
+  void* work = nullptr;  // nd_adjust_bytes(batch)
 };
 
 size_t nd_adjust_bytes(uint32_t batch) {
-  return (size_t)batch * kMaxRecords * sizeof(Record) + ((size_t)batch + 1) * kCounterStride * 4;
+  return kCounterStride * 4 + (size_t)batch * sizeof(RowSpace);
 }
 
 hipError_t nd_launch_adjust(const float* logits, uint32_t batch, uint32_t vocab,
@@ -452,8 +461,7 @@ hipError_t nd_launch_adjust(const float* logits, uint32_t batch, uint32_t vocab,
                             uint32_t* ids, double* logprobs, void* work, hipStream_t s,
                             const nd_select_advance* adv) {
   const uint32_t segments = (vocab + kSegment - 1) / kSegment;
-  Record* records = reinterpret_cast<Record*>(work);
-  uint32_t* counters = reinterpret_cast<uint32_t*>(records + (size_t)batch * kMaxRecords);
+  uint32_t* const rows_done = static_cast<uint32_t*>(work);
   // As few segments a workgroup as let the GPU hold them all at once (three
   // workgroups to a CU, by their LDS), and as few workgroups as that leaves: 100
   // rows of 8 segments take 14.1 us in 4 workgroups a row, 14.3 in 5, 15.5 in 8;
@@ -466,8 +474,9 @@ hipError_t nd_launch_adjust(const float* logits, uint32_t batch, uint32_t vocab,
                 : xl ? (out ? adjust_kernel<true, true, true> : adjust_kernel<true, false, true>)
                      : (out ? adjust_kernel<true, true, false> : adjust_kernel<true, false, false>);
   hipLaunchKernelGGL(kernel, ids && xl ? dim3((batch + 7) / 8 * 8 * S) : dim3(S, batch),
-                     dim3(kThreads), 0, s, logits, vocab, p, mask, out, ids, logprobs, records,
-                     counters, adv ? *adv : nd_select_advance{}, batch, S);
+                     dim3(kThreads), 0, s, logits, vocab, p, mask, out, ids, logprobs,
+                     rows_done, reinterpret_cast<RowSpace*>(rows_done + kCounterStride),
+                     adv ? *adv : nd_select_advance{}, batch, S);
   return hipGetLastError();
 }
 

@@ -374,9 +374,9 @@ hipError_t nd_launch_attention_gated(const nd_kv* kv, uint32_t layer, const uint
 size_t nd_attention_batch_partial_floats(uint32_t batch, uint32_t seq_kv_heads, uint32_t rep,
                                          uint32_t max_count);
 
-// Adjusted selection (adjust.hip): `work` is nd_adjust_bytes(batch) of device
-// memory, zero when first used and left zero where it counts by every launch;
-// launches sharing it must be ordered.  ids == nullptr only writes `out`.
+// Adjusted selection (adjust.hip): `work` is nd_adjust_bytes of this batch or a
+// larger one of device memory, zero when first used and left zero where it counts by
+// every launch; launches sharing it must be ordered.  ids == nullptr only writes `out`.
 size_t nd_adjust_bytes(uint32_t batch);
 hipError_t nd_launch_adjust(const float* logits, uint32_t batch, uint32_t vocab,
                             const nd_logit_adjust& p, const uint32_t* mask, float* out,

@@ -1,0 +1,95 @@
+"""Calls of the shared-prompt operators that follow one another on one handle, and
+arguments at the ends of their ranges, against plain models.
+
+Bars.  Ids, adjusted logits and products are exact by definition.  A
+log-probability is a float64 sum whose terms e^x are each off by at most 4e-11
+of themselves; a term is scaled by such a factor again when its thread, wave,
+workgroup and row find larger maxima, at most once a segment of 4096 ids of its
+workgroup and three times in the joins, and the float64 sum over v terms rounds
+within v 2^-53: (4 + segments) 4e-11 + v 2^-53, which for the vocabularies here
+(25 segments, of which a workgroup takes at most two: 2.4e-10 and 1.1e-11) stays
+below 2.6e-10, relative to 1 + |log-probability| for its last subtractions.
+"""
+
+import ctypes as C
+import sys
+
+import numpy as np
+import pytest
+
+from helpers import DeviceArray
+from needle_hip import HipSelector
+from needle_hip import lib as L
+from test_gpu_shared import adjusted_oracle, choice_oracle
+
+pytestmark = pytest.mark.gpu
+LP_BAR = 2.6e-10
+
+
+def say(*args):
+    print("[case]", *args, file=sys.stderr, flush=True)
+
+
+class Choice:
+    """One adjusted selection on device arrays, its results filled with values that no
+    selection gives before every call."""
+
+    def __init__(self, rng, rows, v):
+        self.rows, self.v = rows, v
+        self.logits = (rng.standard_normal((rows, v)) * 4).astype(np.float32)
+        self.told = dict(history=rng.integers(0, v, (rows, 90)).astype(np.uint32),
+                         repetition=rng.uniform(1.0, 1.5, rows).astype(np.float32),
+                         frequency=rng.uniform(0.0, 0.5, rows).astype(np.float32))
+        self.dl = DeviceArray(self.logits)
+        self.arrays = {k: DeviceArray(a) for k, a in self.told.items()}
+        self.adjust = L.LogitAdjust()
+        for name, a in self.arrays.items():
+            setattr(self.adjust, name, a.ptr.value)
+        self.adjust.history_stride = 90
+        self.want = [choice_oracle(adjusted_oracle(self.logits, r, self.told), np.ones(v, bool))
+                     for r in range(rows)]
+
+    def run(self, hip, selector):
+        ids = DeviceArray(np.full(self.rows, 0x5A5A5A5A, np.uint32))
+        lps = DeviceArray(np.full(self.rows, 1e300))
+        selector.run(self.dl.ptr.value, self.rows, self.v, ids.ptr.value, lps.ptr.value, self.adjust)
+        hip._check(hip.lib.nd_sync(hip.ctx))
+        got = ids.read(), lps.read()
+        ids.free(), lps.free()
+        return got
+
+    def check(self, got):
+        for r, (pick, lp) in enumerate(self.want):
+            assert got[0][r] == pick, (r, got[0][r], pick)
+            assert abs(got[1][r] - lp) <= LP_BAR * (1 + abs(lp)), (r, got[1][r], lp)
+
+    def free(self):
+        for a in [self.dl, *self.arrays.values()]:
+            a.free()
+
+
+@pytest.mark.parametrize("xcd_local", [True, False])
+def test_one_selector_for_batches_of_changing_size(hip, rng, xcd_local):
+    """A batch that shrinks as its answers end, and grows again: every row of every call is
+    chosen, with the bits of a selector of its own."""
+    say("selector sizes", xcd_local)
+    calls = [Choice(rng, rows, v) for rows, v in
+             ((9, 8192), (4, 8192), (1, 8192), (8, 30000), (9, 30000), (2, 100000), (3, 4097),
+              (64, 32768), (40, 32768), (1, 32768), (5, 100))]
+    probed = C.c_uint32()
+    selector = HipSelector(hip, 70)
+    try:
+        hip._check(hip.lib.nd_test_xcd_local(hip.ctx, int(xcd_local), C.byref(probed)))
+        for turn in (calls, calls[::-1], calls):
+            for call in turn:
+                got = call.run(hip, selector)
+                call.check(got)
+                own = HipSelector(hip, call.rows)
+                alone = call.run(hip, own)
+                own.free()
+                assert np.array_equal(got[0], alone[0]) and np.array_equal(got[1], alone[1])
+    finally:
+        hip._check(hip.lib.nd_test_xcd_local(hip.ctx, 1, C.byref(probed)))
+    selector.free()
+    for call in calls:
+        call.free()
