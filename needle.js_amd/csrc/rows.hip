@@ -608,6 +608,7 @@ nd_status nd_matmul_w8a8(nd_ctx* ctx, const nd_mat* m, const float* x, uint32_t 
   if (st != ND_OK) return st;
   if (rows == 0) return ND_OK;
   if (!x || !y) return nd_fail(ctx, ND_ERR_INVALID, "x or y is NULL");
+  ND_ON_DEVICE(ctx);
   nd_rows* r = nullptr;
   st = nd_rows_create(ctx, rows, m->k, &r);
   if (st != ND_OK) return st;
