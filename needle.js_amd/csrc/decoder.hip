@@ -505,9 +505,10 @@ nd_status nd_batch_create(nd_ctx* ctx, nd_decoder* dec, uint32_t batch, uint32_t
 nd_status nd_batch_free(nd_ctx* ctx, nd_batch* b) {
   if (!ctx) return nd_fail(nullptr, ND_ERR_BACKEND, "context is NULL");
   if (!b) return ND_OK;
+  ND_ON_DEVICE(ctx);
   ND_HIP(ctx, hipStreamSynchronize(ctx->stream));
   if (b->shared || b->adjust_arena) {
-    hipDeviceSynchronize();  // steps may have used any stream
+    ND_HIP(ctx, hipDeviceSynchronize());  // steps may have used any stream
     hipFree(b->shared);
     hipFree(b->adjust_arena);
   }

@@ -66,6 +66,7 @@ call("nd_select_adjusted", lambda: selector.select(x, repetition=np.ones(9)))
 call("nd_selector_free", selector.free)
 call("nd_batch_set_prefix", lambda: batch.set_prefix(prefix, 20))
 call("nd_batch_set_adjust", lambda: batch.set_adjust(8, history=np.zeros((2, 5), np.uint32)))
+call("nd_batch_free", batch.free)
 print(json.dumps(seen))
 """
 
@@ -83,7 +84,7 @@ def seen(tmp_path_factory):
 
 
 WAITS = ("nd_rows_read", "nd_rows_free", "nd_shared_free", "nd_selector_free", "nd_batch_set_prefix",
-         "nd_batch_set_adjust")
+         "nd_batch_set_adjust", "nd_batch_free")
 ENTRIES = ("nd_rows_create", "nd_rows_quantize_d", "nd_matmul_rows_d", "nd_matmul_w8a8",
            "nd_shared_create", "nd_shared_attention_d", "nd_shared_attention", "nd_selector_create",
            "nd_select_adjusted_d", "nd_select_adjusted") + WAITS
