@@ -4,7 +4,8 @@
 // For row r, token v with logit l, c = times v was generated, seen = whether it
 // is anywhere in the row's history (prompt or generated):
 //   a = l;  seen: a = a > 0 ? a / repetition : a * repetition
-//   a = a - frequency c - presence [c > 0] + bias(v)
+//   c > 0: a = a - frequency c - presence
+//   a = a + bias(v)
 // in float64 without contraction, rounded once: the adjusted logits are float32
 // values, as a Float32Array holds them.  bias(v) is the last entry of v in the
 // row's list (Map semantics), 0 without one.  The id and log-probability are
@@ -85,8 +86,10 @@ __device__ __forceinline__ float adjusted(float l, uint32_t counts, bool biased,
   double a = (double)l;
   const uint32_t c = counts & ~kPromptBit;
   if (counts) a = a > 0.0 ? quotient(a, p) : a * p.rep;
-  a = a - p.freq * (double)c;
-  if (c) a = a - p.pres;
+  if (c) {  // an infinite penalty times no occurrence would be NaN
+    a = a - p.freq * (double)c;
+    a = a - p.pres;
+  }
   if (biased) a = a + (double)bias;
   return (float)a;
 }

@@ -20,7 +20,7 @@ import pytest
 from helpers import DeviceArray
 from needle_hip import HipSelector
 from needle_hip import lib as L
-from test_gpu_shared import adjusted_oracle, choice_oracle
+from test_gpu_shared import adjusted_oracle, check_choice, choice_oracle
 
 pytestmark = pytest.mark.gpu
 LP_BAR = 2.6e-10
@@ -93,3 +93,24 @@ def test_one_selector_for_batches_of_changing_size(hip, rng, xcd_local):
     selector.free()
     for call in calls:
         call.free()
+
+
+def test_infinite_penalties_reach_generated_tokens_only(hip, rng):
+    """An infinite frequency or presence penalty bars what was generated and leaves ids of
+    the prompt, of the biases and of no list as they are."""
+    say("infinite penalties")
+    v, n, prompt = 9000, 60, 30
+    logits = (rng.standard_normal((6, v)) * 4).astype(np.float32)
+    history = rng.integers(0, v, (6, n)).astype(np.uint32)
+    history[:, 0] = 0  # the first id is of the prompt
+    history[:, 40] = logits.argmax(1)  # the best one was generated
+    a = dict(history=history, prompt_lengths=np.full(6, prompt, np.uint32),
+             frequency=np.array([np.inf, np.inf, 0.3, -np.inf, np.inf, 0], np.float32),
+             presence=np.array([0.1, np.inf, np.inf, 0, 0, -np.inf], np.float32),
+             bias_ids=rng.integers(0, v, (6, 9)).astype(np.uint32),
+             bias=rng.standard_normal((6, 9)).astype(np.float32))
+    ok = rng.random((6, v)) < 0.3
+    ok[4:, 0] = True
+    with np.errstate(all="ignore"):
+        check_choice(hip, logits, a, None)
+        check_choice(hip, logits, a, ok)
