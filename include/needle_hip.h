@@ -501,7 +501,7 @@ nd_status nd_batch_set_state(nd_ctx* ctx, nd_batch* batch, const uint32_t* token
  * max_position, nd_batch_read, the slots of nd_batch_kv -- count from the end of
  * the prefix: slot i holds position length + i, and attention runs over the
  * prefix and the sequence's own slots (nd_shared_attention_d).  The cache must
- * outlive the steps.  length 0 or prefix NULL gives the batch back positions from
+ * outlive the steps; a step after its end is refused.  length 0 or prefix NULL gives the batch back positions from
  * 0.  Waits for the device; capture steps after it, not before. */
 nd_status nd_batch_set_prefix(nd_ctx* ctx, nd_batch* batch, const nd_kv* prefix, uint32_t length);
 

@@ -757,6 +757,7 @@ nd_status nd_kv_create(nd_ctx* ctx, uint32_t layers, uint32_t kv_heads, uint32_t
     delete kv;
     return st;
   }
+  kv->serial = ++ctx->kv_serial;
   ctx->kvs.insert(kv);
   *out = kv;
   return ND_OK;

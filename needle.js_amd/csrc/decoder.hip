@@ -242,6 +242,7 @@ struct nd_batch {
   // The prompt that every sequence continues (nd_batch_set_prefix): slot i holds
   // position prefix_length + i.
   const nd_kv* prefix = nullptr;
+  uint64_t prefix_serial = 0;  // a later cache may lie at the same address
   uint32_t prefix_length = 0;
   float* shared = nullptr;  // partials of the shared-prefix attention
   // Adjusted selection (nd_batch_set_adjust): one block of device memory with the
@@ -519,7 +520,7 @@ nd_status nd_batch_free(nd_ctx* ctx, nd_batch* b) {
 
 nd_kv* nd_batch_kv(nd_batch* b) { return b ? &b->kv : nullptr; }
 
-// Whether `prefix` (of the context) still holds `length` positions of the
+// Whether `prefix` is a cache of the context that holds `length` positions of the
 // decoder's layers and heads.
 static bool prefix_fits(nd_ctx* ctx, const nd_batch* b, const nd_kv* prefix, uint32_t length) {
   return ctx->kvs.count(const_cast<nd_kv*>(prefix)) && prefix->mode == ND_KV_INT8 &&
@@ -550,6 +551,7 @@ nd_status nd_batch_set_prefix(nd_ctx* ctx, nd_batch* b, const nd_kv* prefix, uin
     ND_HIP(ctx, hipStreamSynchronize(ctx->stream));
   }
   b->prefix = length ? prefix : nullptr;
+  b->prefix_serial = length ? prefix->serial : 0;
   b->prefix_length = length;
   return ND_OK;
 }
@@ -718,7 +720,8 @@ nd_status nd_batch_step(nd_ctx* ctx, nd_batch* b, uint32_t max_position, uint32_
   if (max_position >= b->max_length)
     return nd_fail(ctx, ND_ERR_OVERFLOW, "Position %u reached runtime limit %u", max_position,
                    b->max_length);
-  if (b->prefix_length && !prefix_fits(ctx, b, b->prefix, b->prefix_length))
+  if (b->prefix_length && (!prefix_fits(ctx, b, b->prefix, b->prefix_length) ||
+                           b->prefix->serial != b->prefix_serial))
     return nd_fail(ctx, ND_ERR_INVALID, "the batch's prefix cache is gone");
   hipStream_t s = nd_pick_stream(ctx, stream);
   const nd_decoder* dec = b->dec;

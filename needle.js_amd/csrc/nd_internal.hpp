@@ -48,6 +48,7 @@ struct nd_kv {
   void* v = nullptr;
   float* ks = nullptr;  // [layers][kv_heads][alloc]
   float* vs = nullptr;
+  uint64_t serial = 0;  // of its context's caches: no two have the same (0: a batch's own)
 };
 
 struct nd_ctx {
@@ -80,6 +81,7 @@ struct nd_ctx {
   size_t copy_bytes = 0;  // and take now
   std::set<nd_mat*> mats;
   std::set<nd_kv*> kvs;
+  uint64_t kv_serial = 0;  // of the last cache created
   std::set<nd_pieces*> pieces;
   std::set<nd_grammar*> grammars;
   std::set<nd_rows*> rows;

@@ -18,8 +18,9 @@ import numpy as np
 import pytest
 
 from helpers import DeviceArray
-from needle_hip import HipSelector
+from needle_hip import HipKvCache, HipSelector, NeedleError
 from needle_hip import lib as L
+from needle_hip.models import DecoderGeometry, DecoderWeights, HipBatch, HipDecoder
 from test_gpu_shared import adjusted_oracle, check_choice, choice_oracle
 
 pytestmark = pytest.mark.gpu
@@ -114,3 +115,28 @@ def test_infinite_penalties_reach_generated_tokens_only(hip, rng):
     with np.errstate(all="ignore"):
         check_choice(hip, logits, a, None)
         check_choice(hip, logits, a, ok)
+
+
+def test_batch_knows_its_prefix_cache_from_a_later_one_at_its_address(hip):
+    say("prefix cache replaced")
+    g = DecoderGeometry(layers=2, vocab=512)
+    dec = HipDecoder(hip, DecoderWeights(g, 3))
+    batch = HipBatch(dec, 2, 16)
+    first = HipKvCache(hip, 2, 8, 32)
+    batch.set_prefix(first, 32)
+    batch.set_state([1, 2], [0, 0])
+    batch.step(0)
+    hip._check(hip.lib.nd_sync(hip.ctx))
+    address = first.handle.value
+    first.free()
+    later = []
+    while len(later) < 64 and address not in [c.handle.value for c in later]:
+        later.append(HipKvCache(hip, 2, 8, 32))
+    with pytest.raises(NeedleError) as e:
+        batch.step(1)
+    assert e.value.code == "INVALID_CACT"
+    batch.set_prefix(later[-1], 32)
+    batch.step(1)
+    hip._check(hip.lib.nd_sync(hip.ctx))
+    for x in [batch, dec] + later:
+        x.free()
