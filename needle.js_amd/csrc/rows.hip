@@ -7,8 +7,8 @@
 //
 // The quantizer is the KV cache's own (#storeKV, model/runtime.ts:697-714,
 // 901-907).  The integer sum is exact (k <= 8192, |W c| <= 2^14: below 2^27), so
-// it does not depend on how it is split; the result takes the roundings of
-// (float)sum, two multiplications and the addition.
+// it does not depend on how it is split; the result is add + ((float)sum s_w) s_m with
+// each step rounded to f32, the same bits from every form of the kernels.
 //
 // A handle (nd_rows) holds the quantized rows in the order the matrix cores
 // read, the order of nd_tile_weights: 1 KiB blocks [row / 16][k / 64], lane l of
@@ -151,7 +151,10 @@ struct Four {
     for (int i = 0; i < 4; ++i) s[i] = p.sx[min(m + i, p.M - 1)];
     return s;
   }
+  // Without contraction (here a multiply-add of the second product would take the
+  // place of two roundings in some forms and not in others).
   static __device__ __forceinline__ v4f scaled(v4i c, v4f sw, v4f sx) {
+#pragma clang fp contract(off)
     return v4f{(float)c[0], (float)c[1], (float)c[2], (float)c[3]} * sw * sx;
   }
   // What they are added to (WHOLE: all four are there).

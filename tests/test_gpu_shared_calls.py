@@ -18,10 +18,10 @@ import numpy as np
 import pytest
 
 from helpers import DeviceArray
-from needle_hip import HipKvCache, HipSelector, NeedleError
+from needle_hip import HipKvCache, HipRows, HipSelector, Int8Matrix, NeedleError
 from needle_hip import lib as L
 from needle_hip.models import DecoderGeometry, DecoderWeights, HipBatch, HipDecoder
-from test_gpu_shared import adjusted_oracle, check_choice, choice_oracle
+from test_gpu_shared import adjusted_oracle, check_choice, choice_oracle, quantized
 
 pytestmark = pytest.mark.gpu
 LP_BAR = 2.6e-10
@@ -140,3 +140,32 @@ def test_batch_knows_its_prefix_cache_from_a_later_one_at_its_address(hip):
     hip._check(hip.lib.nd_sync(hip.ctx))
     for x in [batch, dec] + later:
         x.free()
+
+
+# Every form of the product's kernels: few rows, split tiles, whole tiles, k of two blocks.
+@pytest.mark.parametrize("m,n,k", [(1, 301, 4096), (7, 16386, 128), (33, 64, 512), (65, 129, 128),
+                                   (300, 516, 2048), (128, 2048, 256), (64, 16500, 128), (180, 33001, 512),
+                                   (2050, 3088, 512), (2050, 3085, 512), (1025, 1600, 128)])
+def test_products_take_the_roundings_they_are_defined_by(hip, rng, m, n, k):
+    """y = add + ((float)sum s_n) s_m, each step rounded to float32: the same bits from
+    every form."""
+    say("product roundings", m, n, k)
+    w = rng.integers(-128, 128, (n, k)).astype(np.int8)
+    sw = rng.uniform(0.001, 0.02, n).astype(np.float32)
+    x = (rng.standard_normal((m, k)) * rng.uniform(0.01, 10, (m, 1))).astype(np.float32)
+    add = rng.standard_normal((m, n)).astype(np.float32)
+    codes, scales = quantized(x)
+    total = codes.astype(np.float32) @ w.T.astype(np.float32) if k * 2 ** 14 <= 2 ** 24 else (
+        codes.astype(np.float64) @ w.T.astype(np.float64))  # exact either way
+    want = total.astype(np.float32) * sw[None, :] * scales[:, None]
+    mat = hip.upload(Int8Matrix(w, sw.reshape(n, 1), k))
+    rows, dx = HipRows(hip, m, k), DeviceArray(x)
+    rows.quantize(dx.ptr.value, m)
+    y, a = DeviceArray(np.full((m, n), np.nan, np.float32)), DeviceArray(add)
+    rows.matmul(mat, y.ptr.value)
+    rows.matmul(mat, a.ptr.value, add=a.ptr.value)
+    hip._check(hip.lib.nd_sync(hip.ctx))
+    assert np.array_equal(y.read(), want)
+    assert np.array_equal(a.read(), add + want)
+    for d in (dx, y, a, rows):
+        d.free()
