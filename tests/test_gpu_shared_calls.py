@@ -16,9 +16,11 @@ import sys
 
 import numpy as np
 import pytest
+import torch
 
 from helpers import DeviceArray
-from needle_hip import HipKvCache, HipRows, HipSelector, Int8Matrix, NeedleError
+from needle_hip import (HipKvCache, HipRows, HipSelector, HipSharedAttention, Int8Matrix,
+                        NeedleError)
 from needle_hip import lib as L
 from needle_hip.models import DecoderGeometry, DecoderWeights, HipBatch, HipDecoder
 from test_gpu_shared import adjusted_oracle, check_choice, choice_oracle, quantized
@@ -169,3 +171,95 @@ def test_products_take_the_roundings_they_are_defined_by(hip, rng, m, n, k):
     assert np.array_equal(a.read(), add + want)
     for d in (dx, y, a, rows):
         d.free()
+
+
+@pytest.mark.parametrize("v", [1, 2, 3, 5, 31, 32, 33])
+def test_selections_over_the_smallest_vocabularies(hip, rng, v):
+    say("small vocabulary", v)
+    logits = rng.standard_normal((3, v)).astype(np.float32)
+    a = dict(history=rng.integers(0, v + 1, (3, 7)).astype(np.uint32),
+             repetition=np.full(3, 1.5, np.float32), presence=np.full(3, 0.25, np.float32))
+    check_choice(hip, logits, a, None)
+    check_choice(hip, logits, a, np.eye(3, v, dtype=bool))
+
+
+def test_captured_selections_share_a_selector(hip, rng):
+    """Two captured selections of different batches on one selector, replayed in turn with
+    eager ones of a third between them, on one stream: each gives what it gives alone."""
+    say("captured selections")
+    calls = [Choice(rng, rows, v) for rows, v in ((9, 30000), (4, 8192), (6, 20000))]
+    selector = HipSelector(hip, 12)
+    stream = torch.cuda.Stream()
+    outs, graphs = [], []
+    for call in calls:
+        outs.append((torch.zeros(call.rows, dtype=torch.int32, device="cuda"),
+                     torch.zeros(call.rows, dtype=torch.float64, device="cuda")))
+
+    def enqueue(i):
+        call, (ids, lps) = calls[i], outs[i]
+        selector.run(call.dl.ptr.value, call.rows, call.v, ids.data_ptr(), lps.data_ptr(), call.adjust,
+                     stream=stream.cuda_stream)
+
+    torch.cuda.synchronize()
+    for i in range(3):
+        enqueue(i)
+    stream.synchronize()
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            enqueue(i)
+        graphs.append(graph)
+    for turn in range(4):
+        for i in (0, 2, 1, 0, 1, 2):
+            for t in outs[i]:
+                t.fill_(-7)
+            torch.cuda.synchronize()
+            if i < 2:
+                with torch.cuda.stream(stream):
+                    graphs[i].replay()
+            else:
+                enqueue(i)
+            stream.synchronize()
+            calls[i].check([t.cpu().numpy() for t in outs[i]])
+    selector.free()
+    for call in calls:
+        call.free()
+
+
+def test_rows_and_attention_workspaces_take_calls_of_changing_size(hip, rng):
+    """One handle of rows for 40, 1, 17 and 40 rows, one attention workspace for long and
+    short ranges in turn: the bits of handles of their own."""
+    say("workspaces of changing size")
+    k, n = 256, 515
+    w = rng.integers(-127, 128, (n, k)).astype(np.int8)
+    mat = hip.upload(Int8Matrix(w, np.full((n, 1), 0.01, np.float32), k))
+    x = rng.standard_normal((40, k)).astype(np.float32)
+    x[30] = np.inf  # what the larger call leaves behind the smaller one's rows
+    d, y = DeviceArray(x), DeviceArray(np.zeros((40, n), np.float32))
+    rows = HipRows(hip, 40, k)
+
+    def product(handle, m):
+        handle.quantize(d.ptr.value, m)
+        handle.matmul(mat, y.ptr.value)
+        hip._check(hip.lib.nd_sync(hip.ctx))
+        return y.read()[:m]
+
+    for m in (40, 1, 17, 40, 33):
+        got = product(rows, m)
+        own = HipRows(hip, m, k)
+        assert np.array_equal(got, product(own, m), equal_nan=True), m
+        own.free()
+    batch, heads = 20, 2
+    p, o = HipKvCache(hip, 1, heads, 3000), HipKvCache(hip, 1, batch * heads, 500)
+    p.store(0, 0, *rng.standard_normal((2, 3000, heads, 64)).astype(np.float32))
+    o.store(0, 0, *rng.standard_normal((2, 500, batch * heads, 64)).astype(np.float32))
+    q = rng.standard_normal((batch, 2 * heads, 64)).astype(np.float32)
+    shared = HipSharedAttention(hip, batch, heads, 2 * heads)
+    for prefix, longest in ((3000, 500), (10, 1), (0, 0), (3000, 0), (0, 500), (64, 33), (3000, 500)):
+        lengths = np.minimum(longest, rng.integers(0, longest + 1, batch))
+        own = HipSharedAttention(hip, batch, heads, 2 * heads)
+        assert np.array_equal(shared.attention(p, prefix, o, lengths, 0, q),
+                              own.attention(p, prefix, o, lengths, 0, q)), (prefix, longest)
+        own.free()
+    for h in (rows, d, y, shared, p, o):
+        h.free()
