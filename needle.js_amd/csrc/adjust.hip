@@ -99,8 +99,11 @@ __device__ __forceinline__ float adjusted(float l, uint32_t counts, bool biased,
 // its exponent, times the Taylor polynomial of degree 3 (remainder r^4 / 24 <
 // 3.9e-11).  k is the low word of x 64 / ln 2 + 1.5 2^52.  Below -700, and of a NaN (a
 // row whose maximum is NaN or infinite, whose sum is not used), e^x is e^-700: 1e-304
-// in sums of 1 and more.  The sum of a vocabulary's terms keeps the error of 4e-11,
-// and so does a log-probability; the library's exp takes five times the instructions.
+// in sums of 1 and more.  A sum carries 4e-11 from its terms and as much again from
+// every larger maximum that it is scaled to: at most one a segment of its workgroup and
+// three in the joins.  With (4 + segments) 4e-11 at most, it moves a log-probability by
+// 2e-12 to 4e-12 over 8192 to 50001 normal logits; the library's exp takes five times
+// the instructions.
 __device__ __forceinline__ double exp_neg(double x, const double* table) {
   x = fmax(x, -700.0);
   const double shift = 6755399441055744.0, kd = fma(x, 92.33248261689366, shift);
@@ -140,7 +143,7 @@ __device__ __forceinline__ Best wave_best(Best b) {
 }
 
 // SELECT: ids and log-probabilities; STORE: the adjusted logits.  Workgroup
-// (s, r) takes segments s, s + gridDim.x, ... of row r; thread t the ids
+// (s, r) takes segments s, s + S, ... of row r; thread t the ids
 // 4 (t + kThreads i) + [0, 4) of a segment.  XL: the grid is one-dimensional with a
 // row's workgroups on one XCD (workgroup L runs on XCD L % 8), so that records and
 // counters stay in its L2, as in the attention's chunk merge (nd_wave.hpp).
@@ -465,10 +468,12 @@ hipError_t nd_launch_adjust(const float* logits, uint32_t batch, uint32_t vocab,
                             const nd_select_advance* adv) {
   const uint32_t segments = (vocab + kSegment - 1) / kSegment;
   uint32_t* const rows_done = static_cast<uint32_t*>(work);
-  // As few segments a workgroup as let the GPU hold them all at once (three
-  // workgroups to a CU, by their LDS), and as few workgroups as that leaves: 100
-  // rows of 8 segments take 14.1 us in 4 workgroups a row, 14.3 in 5, 15.5 in 8;
-  // 301 rows of 13 take 47.0 in 3, 47.4 in 2, 52.4 in 13.
+  // As few segments a workgroup as would let the GPU hold them all at once (three
+  // workgroups to a CU, by their LDS) if a row's divided evenly, and as few workgroups
+  // a row as that leaves, rounded up: up to twice as many as it holds.  With the logits
+  // in the last-level cache, 100 rows of 8 segments take 14.1 us in 4 workgroups a row
+  // (400 in all), 14.3 in 5, 15.5 in 8; 301 rows of 13 take 47.0 in 3 (903), 47.4 in 2,
+  // 52.4 in 13.  From memory the latter take 53.7 in 3.
   const uint64_t held = 768, each = ((uint64_t)batch * segments + held - 1) / held;
   uint32_t S = (uint32_t)((segments + each - 1) / each);
   if (S > kMaxRecords) S = kMaxRecords;

@@ -1,6 +1,5 @@
-// Token selection shared by the selection kernels (select.hip) and the
-// adjusted selection (adjust.hip): candidate order, JavaScript maximum, the
-// terms of the log-softmax, the advance of a decode batch.
+// What the selection kernels (select.hip) and the adjusted selection (adjust.hip)
+// share: a candidate, and the advance of a decode batch by its selected ids.
 #pragma once
 
 #include "nd_internal.hpp"
@@ -14,42 +13,6 @@ struct Best {
   float v;
   uint32_t order;  // position in candidate order; kNone = no candidate
 };
-
-// True if candidate a should win over b.
-__device__ __forceinline__ bool better(const Best& a, const Best& b) {
-  if (a.order == kNone) return false;
-  if (b.order == kNone) return true;
-  if (a.v > b.v) return true;
-  if (a.v == b.v) return a.order < b.order;
-  if (b.v != b.v) return a.v == a.v;  // NaN best only survives as first candidate (handled by caller)
-  return false;
-}
-
-__device__ __forceinline__ float js_maxf(float a, float b) {
-  if (a != a || b != b) return __builtin_nanf("");
-  return a > b ? a : b;
-}
-
-// One term e^x, x = logit - max <= 0, of the float64 log-softmax sum: the
-// float64 exp while x >= -20, the fast f32 exp below.  The leading term is 1,
-// so the terms below e^-20 = 2.1e-9 together hold at most vocab * 2.1e-9 of
-// the sum.  __expf is v_exp_f32 of x log2(e) rounded to f32: the rounding
-// moves the exponent by at most |x| 1.44 2^-24 (9e-6 at x = -104, where the
-// f32 result reaches 0), i.e. a relative error below 1e-5 with the
-// instruction's own ulp, and flushed subnormals lose terms below 1.2e-38.
-// Together that moves the sum by at most vocab * 2.1e-9 * 1e-5 -- 6.9e-10 at
-// a 32768 vocabulary -- and the log-probability by less than 7e-10.  The float64 exp runs only
-// while some lane of the wave holds such a term, so a row whose logits
-// spread over tens of units (most of the vocabulary below max - 20) costs
-// the f32 exp per term.
-__device__ __forceinline__ double exp_term(float v, double md) {
-  const double x = (double)v - md;
-  double e = (double)__expf((float)x);
-  if (__any(x >= -20.0)) {
-    if (x >= -20.0) e = exp(x);
-  }
-  return e;
-}
 
 }  // namespace sel
 }  // namespace nd
