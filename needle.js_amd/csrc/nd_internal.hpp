@@ -253,8 +253,9 @@ hipError_t nd_launch_attention(const nd_kv* kv, uint32_t layer, uint32_t positio
                                uint32_t stamp_capacity = 0, uint32_t* stamp_workgroups = nullptr);
 hipError_t nd_launch_select_list(const float* logits, uint32_t vocab, const uint32_t* allowed,
                                  uint32_t count, uint32_t* id, double* logprob, hipStream_t s);
-// `split`: nd_select_split_bytes(batch) of device memory, zero when first
-// used and left zero by every launch, that lets each row's vocabulary be
+// `split`: nd_select_split_bytes of this batch or a larger one of device
+// memory, zero when first used and left zero where it counts by every launch,
+// that lets each row's vocabulary be
 // split over several workgroups (vocab % 32 == 0); nullptr keeps one
 // workgroup per row.  Launches sharing one `split` must be ordered.  With
 // `adv` and the split form, the launch also advances a decode batch's state

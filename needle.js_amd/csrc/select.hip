@@ -342,11 +342,20 @@ struct SelRecord {
   double pad;
 };
 static_assert(sizeof(SelRecord) == 32, "record layout");
+// The workspace: the counter of the rows that have advanced in a line of its own, then
+// every row's place, the same whatever the batch of a call, so that calls of any size
+// up to the workspace's may follow one another.
+constexpr uint32_t kSelLine = 32;  // words: 128 bytes
+struct SelSpace {
+  uint32_t arrived;  // workgroups of the row
+  uint32_t pad[kSelLine - 1];
+  SelRecord records[kSelSplitMax];
+};
 
 __global__ __launch_bounds__(kSelectThreads) void select_mask_split_kernel(
     const float* __restrict__ logits_all, uint32_t vocab, const uint32_t* __restrict__ mask_all,
     uint32_t* __restrict__ ids, double* __restrict__ logprobs, uint32_t wps,
-    SelRecord* __restrict__ records, uint32_t* __restrict__ counters, nd_select_advance adv) {
+    uint32_t* __restrict__ rows_done, SelSpace* __restrict__ space, nd_select_advance adv) {
   __shared__ float s_v[16], s_mx[16];
   __shared__ uint32_t s_o[16], s_first[16], s_last;
   __shared__ double s_sum[16];
@@ -405,6 +414,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_mask_split_kernel(
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if (lane == 0) s_sum[w] = sum;
   __syncthreads();
+  SelSpace* const own = space + r;
   if (t == 0) {
     Best best{s_v[0], s_o[0]};
     uint32_t f = s_first[0];
@@ -415,7 +425,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_mask_split_kernel(
       f = min(f, s_first[i]);
       total += s_sum[i];
     }
-    SelRecord* rec = records + (size_t)r * kSelSplitMax + sp;
+    SelRecord* rec = own->records + sp;
     __hip_atomic_store(&rec->bv, best.v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __hip_atomic_store(&rec->bo, best.order, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __hip_atomic_store(&rec->mx, mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -423,16 +433,16 @@ __global__ __launch_bounds__(kSelectThreads) void select_mask_split_kernel(
     __hip_atomic_store(&rec->sum, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __builtin_amdgcn_s_waitcnt(0);  // the record has completed
     const bool last =
-        __hip_atomic_fetch_add(counters + r, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+        __hip_atomic_fetch_add(&own->arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
         S - 1;
-    if (last) __hip_atomic_store(counters + r, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (last) __hip_atomic_store(&own->arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     s_last = last;
   }
   __syncthreads();
   if (!s_last || w != 0) return;
 
   // Merge: lane j holds record j.
-  const SelRecord* rec = records + (size_t)r * kSelSplitMax + (lane < S ? lane : 0);
+  const SelRecord* rec = own->records + (lane < S ? lane : 0);
   float bv = __hip_atomic_load(&rec->bv, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   uint32_t bo = __hip_atomic_load(&rec->bo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   float pm = __hip_atomic_load(&rec->mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -466,7 +476,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_mask_split_kernel(
   ids[r] = id;
   logprobs[r] = lp;
   if (!adv.tokens) return;
-  nd_advance_row(adv, r, gridDim.y, id, lp, counters + gridDim.y);
+  nd_advance_row(adv, r, gridDim.y, id, lp, rows_done);
 }
 
 }  // namespace
@@ -479,7 +489,7 @@ hipError_t nd_launch_select_list(const float* logits, uint32_t vocab, const uint
 }
 
 size_t nd_select_split_bytes(uint32_t batch) {
-  return (size_t)batch * kSelSplitMax * sizeof(SelRecord) + ((size_t)batch + 1) * 4;
+  return kSelLine * 4 + (size_t)batch * sizeof(SelSpace);
 }
 
 hipError_t nd_launch_select_mask(const float* logits, uint32_t batch, uint32_t vocab,
@@ -500,10 +510,10 @@ hipError_t nd_launch_select_mask(const float* logits, uint32_t batch, uint32_t v
     if (S >= 2 && S <= kSelSplitMax) {
       const uint32_t wps = (words + S - 1) / S;
       const uint32_t threads = (wps + 63) / 64 * 64;
-      SelRecord* records = reinterpret_cast<SelRecord*>(split);
-      uint32_t* counters = reinterpret_cast<uint32_t*>(records + (size_t)batch * kSelSplitMax);
+      uint32_t* const rows_done = static_cast<uint32_t*>(split);
       hipLaunchKernelGGL(select_mask_split_kernel, dim3(S, batch), dim3(threads), 0, s, logits,
-                         vocab, mask, ids, logprobs, wps, records, counters,
+                         vocab, mask, ids, logprobs, wps, rows_done,
+                         reinterpret_cast<SelSpace*>(rows_done + kSelLine),
                          adv ? *adv : nd_select_advance{});
       if (advanced) *advanced = adv != nullptr;
       return hipGetLastError();
